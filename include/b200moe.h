@@ -657,7 +657,8 @@ int b200moe_token_logprobs_bwd(const void* logits, int logits_f32, long long ld,
  * counts and types; each tensor fp32 (f32[i] != 0) or bf16, contiguous).
  * grad_partials writes b200moe_grad_partials_count() fp64 partials: sums of
  * squares, or maxima of |g| with inf_norm.  Partials of several calls (other
- * tensors, other ranks) may be added (maximised) elementwise.  grad_clip joins
+ * tensors, other ranks) may be added, or maximised with a maximum that keeps
+ * NaN, elementwise.  grad_clip joins
  * n_partials of them, writes *norm (fp32) and
  * out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)); out[i] may be
  * grads[i].  A norm that is not finite scales by 1.  n = 0 writes the norm

@@ -85,7 +85,12 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, *, shar
     for row, grads in zip(joined, (whole, parts)):
         if grads:
             row.copy_(ops.grad_partials(ops.GradList(grads, "clip_grad_norm_"), inf_norm))
-    dist.all_reduce(joined[1], op=dist.ReduceOp.MAX if inf_norm else dist.ReduceOp.SUM,
-                    group=group)
+    if inf_norm:
+        # The maximum of a reduction may pass over a NaN.  Partials are not negative, so their bits
+        # without the sign, taken as integers, have their order, with a NaN above infinity.
+        bits = joined[1].view(torch.int64).bitwise_and_(2 ** 63 - 1)
+        dist.all_reduce(bits, op=dist.ReduceOp.MAX, group=group)
+    else:
+        dist.all_reduce(joined[1], group=group)
     return ops.grad_clip(every if every.tensors else None, inf_norm, joined.view(-1),
                          float(max_norm))
