@@ -63,25 +63,28 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, *, shar
 
     `sharded`: parameters of which each rank of `group` holds another part (the
     expert-parallel layer's packed experts): their share of the norm is summed over the group,
-    while that of `parameters`, replicated on every rank, counts once.  Parameters
-    without a gradient are left out."""
+    while that of `parameters`, replicated on every rank, counts once.  With a `group` all its
+    ranks make the call, those without sharded parameters too.  Parameters without a gradient
+    are left out."""
     inf_norm = _inf(norm_type)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm!r}")
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    own = list(sharded)
+    parameters, own = list(parameters), list(sharded)
     shards = {id(p) for p in own}
     whole = [p.grad for p in parameters if p.grad is not None and id(p) not in shards]
     parts = [p.grad for p in own if p.grad is not None]
     every = ops.GradList(whole + parts, "clip_grad_norm_")
-    if group is None or not own:
+    if group is None:
         if not every.tensors:
             return torch.zeros(())
         return ops.clip_grads(every, every, inf_norm, float(max_norm))
-    # every rank takes part in the reduction, whether it has gradients or not
+    # every rank takes part in the reduction, whatever it holds
+    held = whole + parts + parameters + own
+    device = held[0].device if held else "cuda" if torch.cuda.is_available() else "cpu"
     count = int(ops._lib.value("b200moe_grad_partials_count"))
-    joined = torch.zeros(2, count, device=own[0].device, dtype=torch.float64)
+    joined = torch.zeros(2, count, device=device, dtype=torch.float64)
     for row, grads in zip(joined, (whole, parts)):
         if grads:
             row.copy_(ops.grad_partials(ops.GradList(grads, "clip_grad_norm_"), inf_norm))

@@ -101,3 +101,29 @@ def test_a_shard_that_is_not_finite_reaches_every_rank(values, norm_type):
     for norm, kept in _run(_nonfinite, values, norm_type):
         assert math.isnan(norm) if nan else norm == math.inf
         assert kept
+
+
+def _uneven(rank, group, nothing_at_all):
+    from spark_gpt_b200 import clip_grad_norm_
+    if rank == 1 and nothing_at_all:
+        return float(clip_grad_norm_([], 1.0, group=group)), []
+    shared = _param(2.0, 4)
+    sharded = [_param(3.0, 9)] if rank == 0 else []
+    norm = clip_grad_norm_((p for p in [shared, *sharded]), 1.0, sharded=sharded, group=group)
+    return float(norm), [float(p.grad[0]) for p in [shared, *sharded]]
+
+
+@pytest.mark.parametrize("nothing_at_all", [False, True])
+def test_a_rank_without_sharded_parameters_takes_part(nothing_at_all):
+    """Its norm and scale hold the other ranks' shards."""
+    (norm, grads), (other, others) = _run(_uneven, nothing_at_all)
+    want = math.sqrt(4 * 4.0 + 9 * 9.0)
+    c = 1.0 / (want + 1e-6)
+    assert math.isclose(norm, want, rel_tol=1e-6)
+    assert math.isclose(grads[0], 2.0 * c, rel_tol=1e-6)
+    assert math.isclose(grads[1], 3.0 * c, rel_tol=1e-6)
+    if nothing_at_all:
+        assert math.isclose(other, 9.0, rel_tol=1e-6)  # it replicates nothing: the shards alone
+    else:
+        assert math.isclose(other, want, rel_tol=1e-6)
+        assert math.isclose(others[0], 2.0 * c, rel_tol=1e-6)
