@@ -69,9 +69,8 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, *, shar
     inf_norm = _inf(norm_type)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm!r}")
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
-    parameters, own = list(parameters), list(sharded)
+    parameters, own = ([p] if isinstance(p, torch.Tensor) else list(p)
+                       for p in (parameters, sharded))
     shards = {id(p) for p in own}
     whole = [p.grad for p in parameters if p.grad is not None and id(p) not in shards]
     parts = [p.grad for p in own if p.grad is not None]

@@ -127,3 +127,18 @@ def test_a_rank_without_sharded_parameters_takes_part(nothing_at_all):
     else:
         assert math.isclose(other, want, rel_tol=1e-6)
         assert math.isclose(others[0], 2.0 * c, rel_tol=1e-6)
+
+
+def _single(rank, group):
+    from spark_gpt_b200 import clip_grad_norm_
+    shard = _param(2.0 + rank, 4)
+    norm = clip_grad_norm_([], 1.0, sharded=shard, group=group)
+    return float(norm), float(shard.grad[0])
+
+
+def test_a_single_sharded_parameter():
+    """Given as itself, as `parameters` may be: not the list of its rows, which have no gradient."""
+    want = math.sqrt(4 * 4.0 + 4 * 9.0)
+    for rank, (norm, grad) in enumerate(_run(_single)):
+        assert math.isclose(norm, want, rel_tol=1e-6)
+        assert math.isclose(grad, (2.0 + rank) / (want + 1e-6), rel_tol=1e-6)
