@@ -162,7 +162,8 @@ class BalancedRouter(nn.Module):
             num_groups=self.num_groups, kept_groups=self.kept_groups,
             group_score=self.group_score, normalize=self.norm_topk_prob, scale=self.scale)
         lead = shape[:-1]
-        return logits.view(*lead, logits.shape[-1]), w.view(*lead, -1), sel.view(*lead, -1)
+        return (logits.view(*lead, logits.shape[-1]), w.view(*lead, self.top_k),
+                sel.view(*lead, self.top_k))
 
     @torch.no_grad()
     def update_bias(self, selected: torch.Tensor, rate: float = 1e-3, group=None) -> None:
@@ -188,4 +189,4 @@ class BalancedSparseMoE(nn.Module):
         logits, w, sel = self.gate(x)
         out = self.experts(x, sel, w)
         lead = shape[:-1]
-        return out.view(shape), logits.view(*lead, -1), sel.view(*lead, -1)
+        return out.view(shape), logits.view(*lead, logits.shape[-1]), sel.view(*lead, sel.shape[-1])
