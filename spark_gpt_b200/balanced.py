@@ -139,7 +139,7 @@ class BalancedRouter(nn.Module):
     Beside TopKRouter's fields the config may hold router_scoring ("sigmoid"), n_group (1),
     topk_group (n_group), router_group_score ("top2") and routed_scaling_factor (1.0), with
     those defaults.  ``score_bias`` is a buffer: it is saved with the model and no
-    optimizer sees it."""
+    optimizer sees it.  It stays fp32 when the module is cast, since bf16 would lose its steps."""
 
     def __init__(self, config):
         super().__init__()
@@ -152,7 +152,14 @@ class BalancedRouter(nn.Module):
         self.group_score = getattr(config, "router_group_score", "top2")
         self.scale = getattr(config, "routed_scaling_factor", 1.0)
         self.weight = nn.Parameter(torch.empty(config.num_experts, config.hidden_size))
-        self.register_buffer("score_bias", torch.zeros(config.num_experts))
+        self.register_buffer("score_bias", torch.zeros(config.num_experts, dtype=torch.float32))
+
+    def _apply(self, fn, recurse=True):
+        bias = self.score_bias
+        super()._apply(fn, recurse)
+        if self.score_bias.dtype != torch.float32:  # moved, and not cast
+            self.score_bias = bias.to(self.score_bias.device)
+        return self
 
     def forward(self, hidden_states: torch.Tensor):
         shape = hidden_states.shape

@@ -44,3 +44,27 @@ def test_balanced_layer_takes_empty_and_ragged_batches(shape):
             assert not p.grad.any()
     if x.numel() == 0:
         assert torch.equal(m.gate.score_bias, before)
+
+
+def test_balanced_layer_cast_to_bf16():
+    """The layer casts its fp32 weights to bf16 itself, so a bf16 module of the same weights gives
+    the same bits, and its bias still moves."""
+    m, h = moe(), moe()
+    with torch.no_grad():
+        for p in m.parameters():
+            p.copy_(p.to(BF16))
+    h.load_state_dict(m.state_dict())
+    h.to(BF16)
+    x = torch.randn(70, 256, device=DEV).to(BF16)
+    dout = torch.randn(70, 256, device=DEV).to(BF16)
+    for a, b in zip(m(x), h(x)):
+        assert torch.equal(a, b)
+    m(x)[0].backward(dout)
+    h(x)[0].backward(dout)
+    for p, q in zip(m.parameters(), h.parameters()):
+        assert q.grad.dtype == BF16
+        if p is m.gate.weight:
+            assert torch.equal(p.grad.to(BF16), q.grad)
+    sel = h(x)[2]
+    h.gate.update_bias(sel, rate=1e-3)
+    assert h.gate.score_bias.dtype == F32 and float(h.gate.score_bias.abs().max()) == pytest.approx(1e-3)

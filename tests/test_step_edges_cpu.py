@@ -40,3 +40,34 @@ def test_batches_without_tokens(layer, lead):
     assert logits.shape == (*lead, 8) and selected.shape == (*lead, 2)
     logits, weights, selected = layer.gate(x)
     assert logits.shape == (*lead, 8) and weights.shape == selected.shape == (*lead, 2)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.bfloat16(),
+                                  lambda m: m.half().bfloat16(), lambda m: m.double()],
+                         ids=["to", "bfloat16", "half", "double"])
+def test_the_selection_bias_stays_fp32(cast):
+    """Its steps of 1e-3 are lost in bf16, and the router takes it in fp32: a cast of the module's
+    parameters leaves its type and values."""
+    from spark_gpt_b200 import BalancedSparseMoE
+    moe = torch.nn.ModuleList([BalancedSparseMoE(CONFIG)])
+    gate = moe[0].gate
+    gate.score_bias.copy_(1.0 + 0.001 * torch.arange(8))
+    want = gate.score_bias.clone()
+    cast(moe)
+    assert gate.weight.dtype != torch.float32
+    assert gate.score_bias.dtype == torch.float32 and torch.equal(gate.score_bias, want)
+    assert set(gate.state_dict()) == {"weight", "score_bias"}
+    moe.to("meta")
+    assert gate.score_bias.device.type == "meta" and gate.score_bias.dtype == torch.float32
+    moe.to_empty(device="cpu")
+    assert gate.score_bias.device.type == "cpu" and gate.score_bias.dtype == torch.float32
+
+
+def test_the_selection_bias_is_fp32_whatever_the_default():
+    from spark_gpt_b200 import BalancedSparseMoE
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        moe = BalancedSparseMoE(CONFIG)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert moe.gate.score_bias.dtype == torch.float32
