@@ -126,7 +126,11 @@ class _RouterLogitsFn(torch.autograd.Function):
         xb, wr = ctx.saved_tensors
         E, W, xdtype, wdtype = ctx.cfg
         faults.raise_pending(xb.device)
-        dl = _extra_logit_grad(d_logits, xb.shape[0], W)
+        if W == E:
+            dl = _extra_logit_grad(d_logits, xb.shape[0], W)
+        else:  # the products take W columns: zeros beyond E, wherever the gradient's rows lie
+            dl = xb.new_zeros(xb.shape[0], W)
+            dl[:, :E] = d_logits
         dx = ops.router_dgrad(dl, wr).to(xdtype) if ctx.needs_input_grad[0] else None
         dw = ops.router_wgrad(xb, dl, E).to(wdtype) if ctx.needs_input_grad[1] else None
         faults.snapshot(xb.device)

@@ -68,3 +68,24 @@ def test_balanced_layer_cast_to_bf16():
     sel = h(x)[2]
     h.gate.update_bias(sel, rate=1e-3)
     assert h.gate.score_bias.dtype == F32 and float(h.gate.score_bias.abs().max()) == pytest.approx(1e-3)
+
+
+@pytest.mark.parametrize("E", [60, 64])
+def test_log_probabilities_of_the_routers_logits(E):
+    """Their gradient's rows lie as the logits' do, W apart: the router's gradients are those of the
+    same gradient in contiguous rows."""
+    import spark_gpt_b200 as b200
+    m = moe(E=E, k=4)
+    x = torch.randn(70, 256, device=DEV).to(BF16)
+    tokens = torch.randint(E, (70,), device=DEV)
+
+    def grads(contiguous):
+        m.zero_grad()
+        xl = x.clone().requires_grad_(True)
+        logits, _, _ = m.gate(xl)
+        r = b200.token_logprobs(logits.contiguous() if contiguous else logits, tokens)
+        (r.entropy - r.logprob).sum().backward()
+        return xl.grad, m.gate.weight.grad
+
+    for a, b in zip(grads(False), grads(True)):
+        assert torch.isfinite(a).all() and torch.equal(a, b)

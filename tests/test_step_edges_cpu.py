@@ -71,3 +71,31 @@ def test_the_selection_bias_is_fp32_whatever_the_default():
     finally:
         torch.set_default_dtype(torch.float32)
     assert moe.gate.score_bias.dtype == torch.float32
+
+
+@pytest.mark.parametrize("E,W", [(60, 64), (8, 8), (1, 8)])
+@pytest.mark.parametrize("stride", ["padded", "contiguous", "wide"])
+def test_logit_gradients_reach_the_router_in_its_width(monkeypatch, E, W, stride):
+    """A gradient whose rows lie W apart (from a padded copy, or of log probabilities of the router's
+    logits) has anything between its rows: the products take W columns, zero beyond E."""
+    from spark_gpt_b200 import balanced, faults, ops
+    seen = {}
+    monkeypatch.setattr(ops, "router_dgrad", lambda dl, wr: seen.setdefault("dgrad", dl) @ wr)
+    monkeypatch.setattr(ops, "router_wgrad", lambda x, dl, E: (seen.setdefault("wgrad", dl).T @ x)[:E])
+    monkeypatch.setattr(faults, "raise_pending", lambda device: None)
+    monkeypatch.setattr(faults, "snapshot", lambda device: None)
+    T, H = 6, 16
+    xb = torch.randn(T, H).to(torch.bfloat16)
+    wr = torch.zeros(W, H, dtype=torch.bfloat16)
+    wr[:E] = torch.randn(E, H)
+    ld = {"padded": W, "contiguous": E, "wide": W + 8}[stride]
+    rows = torch.full((T, ld), float("nan"), dtype=torch.bfloat16)
+    rows[:, :E] = torch.randn(T, E)
+    d = rows[:, :E]
+    ctx = SimpleNamespace(saved_tensors=(xb, wr), cfg=(E, W, torch.bfloat16, torch.float32),
+                          needs_input_grad=(True, True))
+    dx, dw = balanced._RouterLogitsFn.backward(ctx, d)
+    for dl in (seen["dgrad"], seen["wgrad"]):
+        assert dl.shape == (T, W) and dl.is_contiguous() and dl.data_ptr() % 16 == 0
+        assert torch.equal(dl[:, :E], d) and not dl[:, E:].any()
+    assert torch.equal(dx, d.contiguous() @ wr[:E]) and dw.shape == (E, H)
