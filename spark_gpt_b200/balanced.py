@@ -77,7 +77,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | None
     args = (top_k, scoring == "sigmoid", num_groups,
             num_groups if kept_groups is None else kept_groups, group_score == "top2",
             bool(normalize), float(scale))
-    if torch.is_grad_enabled() and rows.requires_grad:
+    if ops.records(rows):
         w, sel = _RouteFn.apply(rows, bias, *args)
     else:
         w, sel = ops.route_experts_fwd(rows, bias, *args)

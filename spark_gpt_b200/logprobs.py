@@ -68,7 +68,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
         raise RuntimeError(f"token_logprobs: need 0 <= top <= min(V, 32), got {top}")
     tokens = tokens.reshape(-1).contiguous()
     args = (rows, tokens, int(top), float(temperature), int(ignore_index))
-    if torch.is_grad_enabled() and rows.requires_grad:
+    if ops.records(rows):
         logprob, entropy, top_lp, top_ids = _TokenLogprobsFn.apply(*args)
     else:
         logprob, entropy, top_lp, top_ids, _ = ops.token_logprobs_fwd(*args, False)

@@ -65,9 +65,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
 
     x: bf16 or fp32 CUDA, any leading dimensions and row stride; weight and bias: of the last
     dimension's size, or None.  The result has x's type and shape."""
-    if torch.is_grad_enabled() and (x.requires_grad
-                                    or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if ops.records(x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, eps)
     rows = ops.aligned_rows(ops.as_rows(x, "layer_norm"))
     y, _ = ops.layer_norm_fwd(rows, _param(weight, rows, "weight"), _param(bias, rows, "bias"), eps,

@@ -14,6 +14,7 @@ from dataclasses import dataclass
 from functools import lru_cache
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib
 
@@ -927,6 +928,18 @@ def route_experts_fwd(logits, bias, top_k, sigmoid, groups, kept, top2, normaliz
     return w, sel
 
 
+def records(*tensors) -> bool:
+    """Whether a call goes through its autograd function: where a gradient is recorded, and inside
+    a forward-mode level, where the function refuses a tangent (the kernels would drop it)."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def refuse_second_order(name: str) -> None:
     """In a backward: grad mode is on there only with create_graph=True, whose graph would lack
     this operator's part."""
@@ -1035,6 +1048,9 @@ class GradList:
                                f"{(set(types) - _GRAD_KINDS.keys()).pop()}")
         if not all(map(torch.Tensor.is_contiguous, tensors)):
             raise RuntimeError(f"{name}: the gradients must be contiguous")
+        if forward_ad._current_level >= 0 and any(
+                forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise RuntimeError(f"{name}: it has no forward-mode derivative")
         self.kinds = array("i", [_GRAD_KINDS[d] for d in types])
         self.ptrs = array("q", list(map(torch.Tensor.data_ptr, tensors)))
         self.sizes = array("q", list(map(torch.Tensor.numel, tensors)))

@@ -99,3 +99,49 @@ def test_logit_gradients_reach_the_router_in_its_width(monkeypatch, E, W, stride
         assert dl.shape == (T, W) and dl.is_contiguous() and dl.data_ptr() % 16 == 0
         assert torch.equal(dl[:, :E], d) and not dl[:, E:].any()
     assert torch.equal(dx, d.contiguous() @ wr[:E]) and dw.shape == (E, H)
+
+
+@pytest.fixture
+def plain_operators(monkeypatch):
+    """The launches replaced by plain forward formulas, so that the calls run on the CPU."""
+    from spark_gpt_b200 import ops
+    monkeypatch.setattr(ops, "as_rows", lambda t, name: t)
+    monkeypatch.setattr(ops, "aligned_rows", lambda t: t)
+    monkeypatch.setattr(ops, "layer_norm_fwd", lambda x, w, b, eps, save, like=None: (
+        torch.nn.functional.layer_norm(x, x.shape[-1:], w, b, eps), x.new_zeros(2, x.shape[0])))
+    monkeypatch.setattr(ops, "route_experts_fwd", lambda x, bias, k, *cfg: torch.topk(torch.sigmoid(x), k))
+    monkeypatch.setattr(ops, "token_logprobs_fwd", lambda x, tokens, *cfg: (
+        x.log_softmax(-1).gather(1, tokens[:, None])[:, 0], x.sum(-1), None, None, x.new_zeros(x.shape[0], 2)))
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+@pytest.mark.parametrize("which", ["norm", "norm weight", "norm bias", "route", "logprob"])
+def test_forward_mode_is_refused(plain_operators, which, grad_mode):
+    """The operators have no forward-mode derivative: a tangent is an error, as it is in the
+    layer, and is not dropped (which would read as zero)."""
+    import torch.autograd.forward_ad as fwd
+
+    import spark_gpt_b200 as b200
+    x, w, b = torch.randn(4, 8), torch.randn(8), torch.randn(8)
+    tokens = torch.zeros(4, dtype=torch.int64)
+    calls = {"norm": lambda f: b200.layer_norm(f(x), w, b), "norm weight": lambda f: b200.layer_norm(x, f(w), b),
+             "norm bias": lambda f: b200.layer_norm(x, w, f(b)), "route": lambda f: b200.route_experts(f(x), 2),
+             "logprob": lambda f: b200.token_logprobs(f(x), tokens)}
+    with torch.set_grad_enabled(grad_mode):
+        calls[which](lambda t: t)
+        with fwd.dual_level():
+            calls[which](lambda t: t)  # without a tangent nothing changes
+            with pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
+                calls[which](lambda t: fwd.make_dual(t, torch.ones_like(t)))
+
+
+def test_gradient_lists_refuse_tangents(monkeypatch):
+    import torch.autograd.forward_ad as fwd
+
+    from spark_gpt_b200 import ops
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    g = torch.randn(4)
+    with fwd.dual_level():
+        ops.GradList([g], "grad_norm")
+        with pytest.raises(RuntimeError, match="grad_norm: .*forward-mode"):
+            ops.GradList([g, fwd.make_dual(g, torch.ones(4))], "grad_norm")
