@@ -658,11 +658,10 @@ int b200moe_token_logprobs_bwd(const void* logits, int logits_f32, long long ld,
  * grad_partials writes b200moe_grad_partials_count() fp64 partials: sums of
  * squares, or maxima of |g| with inf_norm.  Partials of several calls (other
  * tensors, other ranks) may be added, or maximised with a maximum that keeps
- * NaN, elementwise.  grad_clip joins
- * n_partials of them, writes *norm (fp32) and
+ * NaN, elementwise.  grad_clip joins n_partials of them, writes *norm (fp32) and
  * out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)); out[i] may be
- * grads[i].  A norm that is not finite scales by 1.  n = 0 writes the norm
- * alone.  Deterministic. */
+ * grads[i], and shares no memory with another out or gradient.  A norm that
+ * is not finite scales by 1.  n = 0 writes the norm alone.  Deterministic. */
 int b200moe_grad_partials_count(void);
 int b200moe_grad_partials(const void* const* grads, const long long* numel, const int* f32, int n,
                           int inf_norm, double* partials, void* stream);

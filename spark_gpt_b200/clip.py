@@ -37,7 +37,8 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
 @torch.no_grad()
 def clip_grads(grads, max_norm: float, *, out=None, norm_type: float = 2.0) -> torch.Tensor:
     """Scale the gradients by min(1, max_norm / (norm + 1e-6)), in place or into the tensors
-    `out` (same sizes and types); returns the norm before clipping (0-d fp32).
+    `out` (same sizes and types); returns the norm before clipping (0-d fp32).  What is written
+    shares no memory with another tensor of either list.
 
     Where the norm is not finite the gradients keep their values: the caller decides on the
     returned norm whether to take the step."""
@@ -65,14 +66,13 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, *, shar
     expert-parallel layer's packed experts): their share of the norm is summed over the group,
     while that of `parameters`, replicated on every rank, counts once.  With a `group` all its
     ranks make the call, those without sharded parameters too.  Parameters without a gradient
-    are left out."""
+    are left out, and one that is listed twice counts once."""
     inf_norm = _inf(norm_type)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm!r}")
-    parameters, own = ([p] if isinstance(p, torch.Tensor) else list(p)
+    parameters, own = (dict.fromkeys([p] if isinstance(p, torch.Tensor) else p)
                        for p in (parameters, sharded))
-    shards = {id(p) for p in own}
-    whole = [p.grad for p in parameters if p.grad is not None and id(p) not in shards]
+    whole = [p.grad for p in parameters if p.grad is not None and p not in own]
     parts = [p.grad for p in own if p.grad is not None]
     every = ops.GradList(whole + parts, "clip_grad_norm_")
     if group is None:
@@ -80,7 +80,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, *, shar
             return torch.zeros(())
         return ops.clip_grads(every, every, inf_norm, float(max_norm))
     # every rank takes part in the reduction, whatever it holds
-    held = whole + parts + parameters + own
+    held = [*whole, *parts, *parameters, *own]
     device = held[0].device if held else "cuda" if torch.cuda.is_available() else "cpu"
     count = int(ops._lib.value("b200moe_grad_partials_count"))
     joined = torch.zeros(2, count, device=device, dtype=torch.float64)

@@ -7,7 +7,9 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <type_traits>
 
@@ -2405,6 +2407,23 @@ int run_grad_clip(const void* const* grads, void* const* out, const long long* n
   return B200MOE_OK;
 }
 
+int start_grad_partials(const void* const* grads, const long long* numel, const int* f32, int n,
+                        int inf_norm, double* partials, cudaStream_t st) {
+  return n <= kGradTableSmall
+      ? run_grad_partials<kGradTableSmall>(grads, numel, f32, n, inf_norm, partials, st)
+      : run_grad_partials<kGradTableLarge>(grads, numel, f32, n, inf_norm, partials, st);
+}
+
+int start_grad_clip(const void* const* grads, void* const* out, const long long* numel,
+                    const int* f32, int n, int inf_norm, const double* partials, int n_partials,
+                    double max_norm, float* norm, cudaStream_t st) {
+  return n <= kGradTableSmall
+      ? run_grad_clip<kGradTableSmall>(grads, out, numel, f32, n, inf_norm, partials, n_partials,
+                                       max_norm, norm, st)
+      : run_grad_clip<kGradTableLarge>(grads, out, numel, f32, n, inf_norm, partials, n_partials,
+                                       max_norm, norm, st);
+}
+
 int check_grads(const char* what, const void* const* in, const long long* numel, const int* f32,
                 int n) {
   if (n < 0) return fail(B200MOE_ERR_INVALID_ARG, "%s: negative tensor count", what);
@@ -2412,6 +2431,45 @@ int check_grads(const char* what, const void* const* in, const long long* numel,
   for (int i = 0; i < n; ++i) {
     if (numel[i] < 0) return fail(B200MOE_ERR_INVALID_ARG, "%s: tensor %d has a negative size", what, i);
     if (numel[i] && !in[i]) return fail(B200MOE_ERR_INVALID_ARG, "%s: tensor %d is a null pointer", what, i);
+  }
+  return B200MOE_OK;
+}
+
+// The blocks of a clip write without waiting for one another, so no element may be written
+// by two of them, or written by one and read by another: the outputs share no memory with each
+// other or with any gradient but their own, which they cover exactly.
+int check_clip(const char* what, const void* const* in, void* const* out, const long long* numel,
+               const int* f32, int n) {
+  struct Range {
+    uintptr_t lo, hi;
+    int index;
+    bool written;
+  };
+  const std::unique_ptr<Range[]> all(new (std::nothrow) Range[2 * static_cast<size_t>(n) + 1]);
+  if (!all) return fail(B200MOE_ERR_INVALID_ARG, "%s: no host memory for %d tensors", what, n);
+  int m = 0;
+  bool rising = true;
+  for (int i = 0; i < n; ++i) {
+    if (numel[i] == 0) continue;
+    if (!out[i]) return fail(B200MOE_ERR_INVALID_ARG, "%s: output %d is a null pointer", what, i);
+    const uintptr_t bytes = static_cast<uintptr_t>(numel[i]) * (f32[i] ? 4 : 2);
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out[i]), g = reinterpret_cast<uintptr_t>(in[i]);
+    rising = rising && o == g && (m == 0 || all[m - 1].lo <= o);
+    all[m++] = Range{o, o + bytes, i, true};
+    if (o != g) all[m++] = Range{g, g + bytes, i, false};
+  }
+  if (!rising) std::sort(all.get(), all.get() + m, [](const Range& a, const Range& b) { return a.lo < b.lo; });
+  // the range that reaches farthest, of those written and of all
+  const Range* wrote = nullptr;
+  const Range* any = nullptr;
+  for (int j = 0; j < m; ++j) {
+    const Range& r = all[j];
+    const Range* before = r.written ? any : wrote;
+    if (before && before->hi > r.lo)
+      return fail(B200MOE_ERR_INVALID_ARG, "%s: tensors %d and %d overlap where one is written", what,
+                  std::min(before->index, r.index), std::max(before->index, r.index));
+    if (!any || any->hi < r.hi) any = &r;
+    if (r.written && (!wrote || wrote->hi < r.hi)) wrote = &r;
   }
   return B200MOE_OK;
 }
@@ -2710,13 +2768,11 @@ int b200moe_grad_partials_count(void) { return kGradPartials; }
 
 int b200moe_grad_partials(const void* const* grads, const long long* numel, const int* f32, int n,
                           int inf_norm, double* partials, void* stream) {
-  int rc = check_grads("grad_partials", grads, numel, f32, n);
+  const int rc = check_grads("grad_partials", grads, numel, f32, n);
   if (rc) return rc;
   REQUIRE(partials, "grad_partials: null pointer");
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return n <= kGradTableSmall
-      ? run_grad_partials<kGradTableSmall>(grads, numel, f32, n, inf_norm, partials, st)
-      : run_grad_partials<kGradTableLarge>(grads, numel, f32, n, inf_norm, partials, st);
+  return start_grad_partials(grads, numel, f32, n, inf_norm, partials,
+                             static_cast<cudaStream_t>(stream));
 }
 
 int b200moe_grad_clip(const void* const* grads, void* const* out, const long long* numel,
@@ -2726,21 +2782,23 @@ int b200moe_grad_clip(const void* const* grads, void* const* out, const long lon
   if (rc) return rc;
   REQUIRE(partials && norm && (out || n == 0), "grad_clip: null pointer");
   REQUIRE(n_partials >= 0 && max_norm >= 0.0, "grad_clip: max_norm must not be negative");
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return n <= kGradTableSmall
-      ? run_grad_clip<kGradTableSmall>(grads, out, numel, f32, n, inf_norm, partials, n_partials,
-                                       max_norm, norm, st)
-      : run_grad_clip<kGradTableLarge>(grads, out, numel, f32, n, inf_norm, partials, n_partials,
-                                       max_norm, norm, st);
+  if ((rc = check_clip("grad_clip", grads, out, numel, f32, n))) return rc;
+  return start_grad_clip(grads, out, numel, f32, n, inf_norm, partials, n_partials, max_norm, norm,
+                         static_cast<cudaStream_t>(stream));
 }
 
 int b200moe_clip_grads(const void* const* grads, void* const* out, const long long* numel,
                        const int* f32, int n, int inf_norm, double* partials, double max_norm,
                        float* norm, void* stream) {
-  const int rc = b200moe_grad_partials(grads, numel, f32, n, inf_norm, partials, stream);
-  return rc ? rc
-            : b200moe_grad_clip(grads, out, numel, f32, n, inf_norm, partials, kGradPartials, max_norm,
-                                norm, stream);
+  int rc = check_grads("clip_grads", grads, numel, f32, n);
+  if (rc) return rc;
+  REQUIRE(partials && norm && (out || n == 0), "clip_grads: null pointer");
+  REQUIRE(max_norm >= 0.0, "clip_grads: max_norm must not be negative");
+  if ((rc = check_clip("clip_grads", grads, out, numel, f32, n))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = start_grad_partials(grads, numel, f32, n, inf_norm, partials, st))) return rc;
+  return start_grad_clip(grads, out, numel, f32, n, inf_norm, partials, kGradPartials, max_norm, norm,
+                         st);
 }
 
 }  // extern "C"

@@ -89,3 +89,26 @@ def test_log_probabilities_of_the_routers_logits(E):
 
     for a, b in zip(grads(False), grads(True)):
         assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_gradients_side_by_side_are_clipped_and_shared_ones_refused():
+    """Neighbours in one buffer, in any order, share no memory; a tensor that is read twice may be."""
+    import spark_gpt_b200 as b200
+    big = torch.ones(3000, device=DEV)
+    parts = [big[2000:], big[:999], big[999:2000], big[5:5]]
+    norm = b200.clip_grads(parts, 1.0)
+    assert float(norm) == pytest.approx(3000 ** 0.5)
+    assert torch.allclose(big, big.new_tensor(3000 ** -0.5).expand(3000), rtol=1e-6)
+    g, out = torch.ones(8, device=DEV), torch.zeros(16, device=DEV)
+    assert float(b200.grad_norm([g, g])) == 4.0
+    assert float(b200.clip_grads([g, g], 2.0, out=[out[:8], out[8:]])) == 4.0
+    assert torch.allclose(out, torch.full_like(out, 0.5), rtol=1e-6) and bool((g == 1).all())
+    for grads, o in (([g, g], None), ([g[:5], g[4:]], None), ([g[:4], g[4:]], [g[4:], g[:4]]),
+                     ([g, g], [out[:8], out[7:15]])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            b200.clip_grads(grads, 0.5, out=o)
+    assert bool((g == 1).all())
+    p = torch.nn.Parameter(torch.zeros(4, device=DEV))
+    p.grad = torch.ones(4, device=DEV)
+    assert float(b200.clip_grad_norm_([p, p], 1.0)) == 2.0
+    assert torch.allclose(p.grad, torch.full_like(p.grad, 0.5), rtol=1e-6)

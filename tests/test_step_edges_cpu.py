@@ -145,3 +145,51 @@ def test_gradient_lists_refuse_tangents(monkeypatch):
         ops.GradList([g], "grad_norm")
         with pytest.raises(RuntimeError, match="grad_norm: .*forward-mode"):
             ops.GradList([g, fwd.make_dual(g, torch.ones(4))], "grad_norm")
+
+
+@pytest.fixture(scope="module")
+def call():
+    from spark_gpt_b200 import _lib
+    from spark_gpt_b200.build import build
+    build()
+    return _lib.call
+
+
+MiB = 1 << 20
+
+
+@pytest.mark.parametrize("entry", ["b200moe_grad_clip", "b200moe_clip_grads"])
+@pytest.mark.parametrize("grads,out,sizes,kinds", [
+    ([MiB, MiB], None, [8, 8], [1, 1]),                           # the same tensor twice
+    ([MiB, 2 * MiB, 3 * MiB, MiB], None, [8, 8, 8, 4], [1] * 4),  # again, with others between
+    ([MiB, MiB + 12], None, [4, 8], [1, 1]),                      # an end in the next one's start
+    ([2 * MiB, MiB], None, [4, MiB // 4 + 1], [1, 1]),            # the same in falling order
+    ([MiB, MiB + 64, MiB + 128], None, [1000, 2, 2], [0, 0, 0]),  # two inside a first
+    ([MiB, 2 * MiB], [3 * MiB, 3 * MiB + 8], [8, 8], [0, 0]),     # outputs into each other
+    ([MiB, 2 * MiB], [3 * MiB, MiB], [8, 8], [1, 1]),             # an output into another gradient
+    ([MiB], [MiB + 4], [8], [1]),                                 # into its own, shifted
+    ([MiB, MiB], [MiB, 2 * MiB], [8, 8], [1, 1]),                 # one read, the same written
+], ids=str)
+def test_gradients_that_share_memory_are_refused(call, entry, grads, out, sizes, kinds):
+    """Blocks that scale them would write the same elements.  Nothing is launched."""
+    from array import array
+    g, o, n, f = array("q", grads), array("q", out or grads), array("q", sizes), array("i", kinds)
+    at = lambda a: a.buffer_info()[0]  # noqa: E731
+    tail = (16, 592, 1.0, 16, None) if entry == "b200moe_grad_clip" else (16, 1.0, 16, None)
+    with pytest.raises(RuntimeError, match="overlap"):
+        call(entry, at(g), at(o), at(n), at(f), len(grads), 0, *tail)
+
+
+def test_a_parameter_listed_twice_counts_once(monkeypatch):
+    """Tied weights reach a list of parameters by two names; the gradient is one."""
+    import spark_gpt_b200 as b200
+    from spark_gpt_b200 import ops
+    seen = []
+    monkeypatch.setattr(ops, "GradList", lambda tensors, name: SimpleNamespace(tensors=tensors))
+    monkeypatch.setattr(ops, "clip_grads", lambda g, out, inf, m: seen.append(g.tensors))
+    a, b, c = (torch.nn.Parameter(torch.zeros(3)) for _ in range(3))
+    for p in (a, b, c):
+        p.grad = torch.ones(3)
+    b200.clip_grad_norm_([a, b, a, c, b], 1.0)
+    b200.clip_grad_norm_([a, b, a], 1.0, sharded=[c, a, c])
+    assert [[id(t) for t in s] for s in seen] == [[id(p.grad) for p in (a, b, c)], [id(p.grad) for p in (b, c, a)]]
