@@ -2690,7 +2690,8 @@ int b200moe_token_logprobs_fwd(const void* logits, int logits_f32, long long ld,
   REQUIRE(T >= 0 && V >= 1 && V <= (1 << 30), "token_logprobs_fwd: need T >= 0 and V >= 1, V <= 2^30");
   REQUIRE(top >= 0 && top <= kMaxAlternatives && top <= V,
           "token_logprobs_fwd: need 0 <= top <= min(V, 32)");
-  REQUIRE(temperature > 0.f, "token_logprobs_fwd: the temperature must be positive");
+  REQUIRE(temperature >= kLeastTemperature && temperature <= kMostTemperature,
+          "token_logprobs_fwd: the temperature must be positive, from 1e-30 to 1e20");
   if (T == 0) return B200MOE_OK;
   REQUIRE(logits && tokens && logprob && entropy && (!top || (top_logprobs && top_ids)),
           "token_logprobs_fwd: null pointer");
@@ -2737,7 +2738,8 @@ int b200moe_token_logprobs_bwd(const void* logits, int logits_f32, long long ld,
                                const float* d_logprob, const float* d_entropy, void* d_logits,
                                long long ld_out, void* stream) {
   REQUIRE(T >= 0 && V >= 1 && V <= (1 << 30), "token_logprobs_bwd: need T >= 0 and V >= 1, V <= 2^30");
-  REQUIRE(temperature > 0.f, "token_logprobs_bwd: the temperature must be positive");
+  REQUIRE(temperature >= kLeastTemperature && temperature <= kMostTemperature,
+          "token_logprobs_bwd: the temperature must be positive, from 1e-30 to 1e20");
   if (T == 0) return B200MOE_OK;
   REQUIRE(logits && tokens && stats && entropy && d_logits, "token_logprobs_bwd: null pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -47,9 +47,12 @@ constexpr float kUnderflow = -200.f;     // 2^-200 is 0 in fp32
 constexpr float kFloorShift = 1e8f;
 constexpr float kLargestShift = 5e7f;    // far enough above the floor that 2^(floor c - m c) is 0
 
+// In this range of temperatures c, 1 / temperature and the floor (-7e-23 to -7e27) are normal numbers.
+constexpr float kLeastTemperature = 1e-30f, kMostTemperature = 1e20f;
+
 // The floor for a scale c: a number of 8 significant bits, so that it is the same in bf16.
 inline float logit_floor(float c) {
-  const float f = fminf(kFloorShift / c, 1e30f);
+  const float f = kFloorShift / c;
   uint32_t b;
   memcpy(&b, &f, 4);
   b &= 0xffff0000u;

@@ -50,7 +50,8 @@ class _TokenLogprobsFn(torch.autograd.Function):
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
                    temperature: float = 1.0, ignore_index: int = -100) -> TokenLogprobs:
-    """logits (..., V) bf16 or fp32, tokens (...) int64, over softmax(logits / temperature).
+    """logits (..., V) bf16 or fp32, tokens (...) int64, over softmax(logits / temperature), the
+    temperature from 1e-30 to 1e20.
 
     Differentiable in the logits through logprob and entropy; the alternatives (the `top` <= 32
     largest logits, equal ones by rising id) are reported only.  A row whose token is

@@ -193,3 +193,16 @@ def test_a_parameter_listed_twice_counts_once(monkeypatch):
     b200.clip_grad_norm_([a, b, a, c, b], 1.0)
     b200.clip_grad_norm_([a, b, a], 1.0, sharded=[c, a, c])
     assert [[id(t) for t in s] for s in seen] == [[id(p.grad) for p in (a, b, c)], [id(p.grad) for p in (b, c, a)]]
+
+
+@pytest.mark.parametrize("temperature", [1e21, 1e30, 3e38, float("inf"), 1e-31, 1e-38, 1e-42, 0.0, -1.0,
+                                         float("nan")])
+def test_temperatures_beyond_the_arithmetic_are_refused(call, temperature):
+    """From 1e-30 to 1e20 the scales and their products with the floor of the logits are fp32 numbers;
+    beyond, a padding place or a -inf logit would have probability."""
+    with pytest.raises(RuntimeError, match="temperature"):
+        call("b200moe_token_logprobs_fwd", 16, 0, 100, 16, 4, 100, temperature, -100, 0, 16, 16, None, None,
+             None, None)
+    with pytest.raises(RuntimeError, match="temperature"):
+        call("b200moe_token_logprobs_bwd", 16, 0, 100, 16, 4, 100, temperature, -100, 16, 16, 16, 16, 16, 100,
+             None)
