@@ -584,7 +584,7 @@ int b200moe_lb_grad(const void* logits, long long ld, const unsigned char* valid
  * Rows are fp32 (`*_f32` != 0) or bf16, `ld` elements apart (ld 0 repeats one
  * row); no alignment beyond the element's own is needed.  T = 0 is valid. */
 
-/* Layer norm: y (T, H) contiguous, of x's type; w, b (H) fp32 or NULL; mean
+/* Layer norm, H <= 2^31 - 1024: y (T, H) contiguous, of x's type; w, b (H) fp32 or NULL; mean
  * and rstd (T) fp32, both NULL when no backward follows. */
 int b200moe_layer_norm_fwd(const void* x, int x_f32, long long ld, const float* w, const float* b,
                            long long T, int H, float eps, void* y, float* mean, float* rstd,

@@ -2265,6 +2265,7 @@ namespace {
   else if ((H) <= 512 * 24) { constexpr int G = 512, NE = 24; __VA_ARGS__ }       \
   else { constexpr int G = 512, NE = 32; __VA_ARGS__ }
 constexpr int kNormMaxCols = 512 * 32;
+constexpr int kNormMostCols = 0x7fffffff - 1023;  // a column and a block's stride fit 32 bits
 
 // Blocks of the backward kernels, each of which writes one row of weight-gradient partials: as
 // many as are resident at once.
@@ -2480,7 +2481,8 @@ extern "C" {
 int b200moe_layer_norm_fwd(const void* x, int x_f32, long long ld, const float* w, const float* b,
                            long long T, int H, float eps, void* y, float* mean, float* rstd,
                            void* stream) {
-  REQUIRE(T >= 0 && H >= 1, "layer_norm_fwd: need T >= 0 and H >= 1");
+  REQUIRE(T >= 0 && H >= 1 && H <= kNormMostCols,
+          "layer_norm_fwd: need T >= 0, H >= 1 and H <= 2^31 - 1024");
   if (T == 0) return B200MOE_OK;
   REQUIRE(x && y && (!mean == !rstd), "layer_norm_fwd: null pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -2525,7 +2527,8 @@ int b200moe_layer_norm_bwd(const void* dy, long long ld_dy, const void* x, int x
                            const float* w, const float* mean, const float* rstd, long long T,
                            int H, void* dx, float* dw, float* db, void* scratch,
                            long long scratch_bytes, void* stream) {
-  REQUIRE(T >= 0 && H >= 1, "layer_norm_bwd: need T >= 0 and H >= 1");
+  REQUIRE(T >= 0 && H >= 1 && H <= kNormMostCols,
+          "layer_norm_bwd: need T >= 0, H >= 1 and H <= 2^31 - 1024");
   REQUIRE(!dw == !db, "layer_norm_bwd: dw and db go together");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (T == 0) {
@@ -2578,7 +2581,7 @@ int b200moe_layer_norm_bwd(const void* dy, long long ld_dy, const void* x, int x
       }
     }
     if (dw) {
-      layer_norm_dw_sum_kernel<<<(2 * H + 31) / 32, kNormThreads, 0, st>>>(part, parts, H, dw, db);
+      layer_norm_dw_sum_kernel<<<static_cast<unsigned>((2LL * H + 31) / 32), kNormThreads, 0, st>>>(part, parts, H, dw, db);
       rc = check_launch("layer_norm_dw_sum");
     }
     return rc;

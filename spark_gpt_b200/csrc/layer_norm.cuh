@@ -692,9 +692,9 @@ layer_norm_dw_kernel(const T* __restrict__ dy, long long ld_dy, const T* __restr
     sw = fmaf(g, (to_f32(x[t * ld + c]) - mean[t]) * rstd[t], sw);
     sb += g;
   }
-  float* p = part + static_cast<long long>(blockIdx.y) * 2 * H;
-  p[c] = sw;
-  p[H + c] = sb;
+  float* p = part + 2LL * blockIdx.y * H + c;  // 2 H may pass 32 bits
+  p[0] = sw;
+  p[static_cast<long long>(H)] = sb;
 }
 
 // dw, db: the partials summed in a fixed order, 32 columns a block, eight threads a column.
@@ -703,15 +703,15 @@ layer_norm_dw_sum_kernel(const float* __restrict__ part, int parts, int H, float
                          float* __restrict__ db) {
   __shared__ float sh[8][32];
   const int lane = threadIdx.x & 31, q = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
+  const long long c = blockIdx.x * 32LL + lane;
   float s = 0.f;
-  if (c < 2 * H) {
+  if (c < 2LL * H) {
 #pragma unroll 4
-    for (int p = q; p < parts; p += 8) s += part[static_cast<long long>(p) * 2 * H + c];
+    for (int p = q; p < parts; p += 8) s += part[2LL * p * H + c];
   }
   sh[q][lane] = s;
   __syncthreads();
-  if (q || c >= 2 * H) return;
+  if (q || c >= 2LL * H) return;
 #pragma unroll
   for (int i = 1; i < 8; ++i) s += sh[i][lane];
   if (c < H) dw[c] = s;

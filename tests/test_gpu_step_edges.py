@@ -112,3 +112,15 @@ def test_gradients_side_by_side_are_clipped_and_shared_ones_refused():
     p.grad = torch.ones(4, device=DEV)
     assert float(b200.clip_grad_norm_([p, p], 1.0)) == 2.0
     assert torch.allclose(p.grad, torch.full_like(p.grad, 0.5), rtol=1e-6)
+
+
+def test_weight_gradients_of_more_columns_than_half_an_int():
+    """2 H passes 31 bits: the weight gradients of one row are products, and found at every column."""
+    from spark_gpt_b200 import ops
+    H = (1 << 30) + 8
+    x = (torch.arange(H, device=DEV, dtype=torch.int32) % 251).to(BF16)[None]
+    dy = (torch.arange(H, device=DEV, dtype=torch.int32) % 127).to(BF16)[None]
+    stats = torch.tensor([[64.0], [0.5]], device=DEV)
+    _, dw, db = ops.layer_norm_bwd(dy, x, None, stats, False, True)
+    assert torch.equal(db, dy[0].float())
+    assert torch.equal(dw, (x[0].float() - 64.0) * 0.5 * dy[0].float())
