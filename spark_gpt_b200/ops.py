@@ -819,9 +819,9 @@ def as_rows(t: torch.Tensor, name: str) -> torch.Tensor:
         raise RuntimeError(f"{name}: the B200 MoE kernels need CUDA tensors (no CPU path)")
     if t.dtype not in (BF16, torch.float32):
         raise RuntimeError(f"{name}: expected bf16 or fp32, got {t.dtype}")
-    if t.dim() == 0 or t.shape[-1] == 0:
-        raise RuntimeError(f"{name}: expected rows of one column or more, got shape "
-                           f"{tuple(t.shape)}")
+    if t.dim() == 0 or not 0 < t.shape[-1] < 2 ** 31:
+        raise RuntimeError(f"{name}: expected rows of one column or more and fewer than 2^31 columns, "
+                           f"got shape {tuple(t.shape)}")
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()

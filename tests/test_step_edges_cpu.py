@@ -206,3 +206,21 @@ def test_temperatures_beyond_the_arithmetic_are_refused(call, temperature):
     with pytest.raises(RuntimeError, match="temperature"):
         call("b200moe_token_logprobs_bwd", 16, 0, 100, 16, 4, 100, temperature, -100, 16, 16, 16, 16, 16, 100,
              None)
+
+
+@pytest.mark.parametrize("columns", [2 ** 31 - 1, 2 ** 31, 2 ** 32 + 8])
+def test_more_columns_than_an_int_holds_are_refused(call, columns):
+    """The entry points take the columns as 32 bits, in which 2^32 + 8 would be 8."""
+    from spark_gpt_b200 import ops
+    rows = SimpleNamespace(is_cuda=True, dtype=torch.bfloat16, shape=(1, columns), dim=lambda: 2,
+                           stride=lambda d: (columns, 1)[d])
+    if columns < 2 ** 31:
+        assert ops.as_rows(rows, "norm") is rows
+        with pytest.raises(RuntimeError, match="H <="):
+            call("b200moe_layer_norm_fwd", 16, 0, columns, None, None, 1, columns, 1e-5, 16, None, None, None)
+        with pytest.raises(RuntimeError, match="H <="):
+            call("b200moe_layer_norm_bwd", 16, columns, 16, 0, columns, None, 16, 16, 1, columns, 16, None,
+                 None, None, 0, None)
+    else:
+        with pytest.raises(RuntimeError, match="norm: .*columns"):
+            ops.as_rows(rows, "norm")
