@@ -634,7 +634,8 @@ int b200moe_balance_step(const long long* selected, long long n, int E, const fl
 /* Log probabilities of tokens (T) under softmax(logits (T, V) / temperature),
  * temperature from 1e-30 to 1e20, the entropy of each row, and with top > 0
  * (<= 32) the `top` largest entries: top_logprobs (T, top), top_ids (T, top),
- * equal values by rising id.  stats (T, 2): what the backward needs, or NULL.
+ * equal values by rising id.  stats (T, 2), on 8 bytes: what the backward
+ * needs, or NULL.
  * A row whose token is `ignore` is left out (0, 0, alternatives 0 and -1); any
  * other token outside [0, V) gives NaN.  A -inf logit has probability 0; a row
  * of -inf alone has entropy 0, log probabilities -inf and gradient 0. */

@@ -2698,6 +2698,7 @@ int b200moe_token_logprobs_fwd(const void* logits, int logits_f32, long long ld,
   if (T == 0) return B200MOE_OK;
   REQUIRE(logits && tokens && logprob && entropy && (!top || (top_logprobs && top_ids)),
           "token_logprobs_fwd: null pointer");
+  REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, "token_logprobs_fwd: stats must lie on 8 bytes");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const float c = 1.4426950408889634f / temperature;
   auto launch = [&](auto zero) -> int {
@@ -2745,6 +2746,7 @@ int b200moe_token_logprobs_bwd(const void* logits, int logits_f32, long long ld,
           "token_logprobs_bwd: the temperature must be positive, from 1e-30 to 1e20");
   if (T == 0) return B200MOE_OK;
   REQUIRE(logits && tokens && stats && entropy && d_logits, "token_logprobs_bwd: null pointer");
+  REQUIRE(reinterpret_cast<uintptr_t>(stats) % 8 == 0, "token_logprobs_bwd: stats must lie on 8 bytes");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const float c = 1.4426950408889634f / temperature;
   auto launch = [&](auto zero) {

@@ -224,3 +224,11 @@ def test_more_columns_than_an_int_holds_are_refused(call, columns):
     else:
         with pytest.raises(RuntimeError, match="norm: .*columns"):
             ops.as_rows(rows, "norm")
+
+
+def test_statistics_off_their_alignment_are_refused(call):
+    """The log probabilities' statistics are read and written as pairs of fp32."""
+    with pytest.raises(RuntimeError, match="stats"):
+        call("b200moe_token_logprobs_fwd", 16, 0, 100, 16, 4, 100, 1.0, -100, 0, 16, 16, None, None, 20, None)
+    with pytest.raises(RuntimeError, match="stats"):
+        call("b200moe_token_logprobs_bwd", 16, 0, 100, 16, 4, 100, 1.0, -100, 20, 16, 16, 16, 16, 100, None)
