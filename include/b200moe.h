@@ -635,10 +635,10 @@ int b200moe_balance_step(const long long* selected, long long n, int E, const fl
  * temperature from 1e-30 to 1e20, the entropy of each row, and with top > 0
  * (<= 32) the `top` largest entries: top_logprobs (T, top), top_ids (T, top),
  * equal values by rising id.  stats (T, 2), on 8 bytes: what the backward
- * needs, or NULL.
- * A row whose token is `ignore` is left out (0, 0, alternatives 0 and -1); any
- * other token outside [0, V) gives NaN.  A -inf logit has probability 0; a row
- * of -inf alone has entropy 0, log probabilities -inf and gradient 0. */
+ * needs, or NULL.  A row whose token is `ignore` is left out (0, 0,
+ * alternatives 0 and -1); any other token outside [0, V) gives NaN.  A -inf
+ * logit has probability 0; a row of -inf alone has entropy 0, log probabilities
+ * -inf and gradient 0. */
 int b200moe_token_logprobs_fwd(const void* logits, int logits_f32, long long ld,
                                const long long* tokens, long long T, int V, float temperature,
                                long long ignore, int top, float* logprob, float* entropy,
