@@ -77,13 +77,26 @@ __device__ __forceinline__ float rcp_approx(float v) {  // 1 ulp; 0 below 2^-126
   return r;
 }
 
+// 1 / (1 + e^-x) below kSmallLogit is e^x (to one part in 10^37), which keeps the scores below 2^-126
+// that the reciprocal makes 0.
+constexpr float kSmallLogit = -87.f;
+__device__ __forceinline__ float sigmoid_score(float x) {
+  return x < kSmallLogit ? expf(x) : rcp_approx(1.0f + expf(-x));
+}
+
 // Scores of a lane's experts (z: its logits, -inf beyond E).  expf, since the selection hangs on
-// them; the reciprocals are within 1 ulp.  A row of -inf alone has softmax scores 0.
+// them; the reciprocals are within 1 ulp.  `small`: with the sigmoid scores below 2^-126.  A row of
+// -inf alone has softmax scores 0.
 template <int L>
-__device__ __forceinline__ void route_scores(float (&z)[kVpt], bool sigmoid) {
+__device__ __forceinline__ void route_scores(float (&z)[kVpt], bool sigmoid, bool small) {
   if (sigmoid) {
+    if (small) {
 #pragma unroll
-    for (int j = 0; j < kVpt; ++j) z[j] = rcp_approx(1.0f + expf(-z[j]));
+      for (int j = 0; j < kVpt; ++j) z[j] = sigmoid_score(z[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVpt; ++j) z[j] = rcp_approx(1.0f + expf(-z[j]));
+    }
     return;
   }
   float m = -INFINITY;
@@ -155,13 +168,14 @@ route_experts_fwd_kernel(const T* __restrict__ logits, long long ld, long long r
 #pragma unroll
   for (int j = 0; j < kVpt; ++j) bs[j] = bias && e0 + j < E ? bias[e0 + j] : 0.f;
   const GroupTokens gt = GroupTokens::make<L>(rows);
-  for (long long rnd = 0; rnd < gt.rounds; ++rnd) {
+  bool small = false;  // the round is done again, with the scores below 2^-126
+  for (long long rnd = 0; rnd < gt.rounds;) {
     const long long t = gt.first + rnd * gt.stride;
     const bool valid = t < rows;
     float s[kVpt];
     int key[kVpt];
     load_chunk(logits + (valid ? t : 0) * ld, e0, E, valid, vec != 0, s);
-    route_scores<L>(s, sigmoid != 0);
+    route_scores<L>(s, sigmoid != 0, small);
 #pragma unroll
     for (int j = 0; j < kVpt; ++j) key[j] = e0 + j < E ? select_key(s[j] + bs[j]) : kTaken;
     if (bias) {  // the winners' scores without the bias are read from here
@@ -291,6 +305,19 @@ route_experts_fwd_kernel(const T* __restrict__ logits, long long ld, long long r
         if (won_r[q] < k) won_s[q] = bias ? sh_s[tok][won_e[q]] : select_value(won_k[q]);
       }
     }
+    // A score that the reciprocal makes 0 changes the outcome only where it is chosen.
+    if (sigmoid && !small) {
+      bool zero = false;
+#pragma unroll
+      for (int q = 0; q < SLOTS; ++q) zero |= valid && won_r[q] < k && won_s[q] == 0.f;
+      small = __any_sync(0xffffffffu, zero);
+      if (small) {
+        __syncwarp();
+        continue;
+      }
+    }
+    small = false;
+    ++rnd;
     float f = scale;
     if (normalize) {
       float total = 0.f;
@@ -332,7 +359,7 @@ route_experts_bwd_kernel(const T* __restrict__ logits, long long ld,
     float s[kVpt];
     if (!sigmoid) {
       load_chunk(row, e0, E, valid, vec != 0, s);
-      route_scores<L>(s, false);
+      route_scores<L>(s, false, false);
       *reinterpret_cast<float4*>(&sh_s[tok][e0]) = make_float4(s[0], s[1], s[2], s[3]);
       *reinterpret_cast<float4*>(&sh_s[tok][e0 + 4]) = make_float4(s[4], s[5], s[6], s[7]);
     }
@@ -357,7 +384,7 @@ route_experts_bwd_kernel(const T* __restrict__ logits, long long ld,
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) {
       if (e[q] >= 0)
-        p[q] = sigmoid ? rcp_approx(1.0f + expf(-to_f32(row[e[q]]))) : sh_s[tok][e[q]];
+        p[q] = sigmoid ? sigmoid_score(to_f32(row[e[q]])) : sh_s[tok][e[q]];
       total += p[q];
       dot = fmaf(dw[q], p[q], dot);
     }

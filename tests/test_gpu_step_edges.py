@@ -124,3 +124,35 @@ def test_weight_gradients_of_more_columns_than_half_an_int():
     _, dw, db = ops.layer_norm_bwd(dy, x, None, stats, False, True)
     assert torch.equal(db, dy[0].float())
     assert torch.equal(dw, (x[0].float() - 64.0) * 0.5 * dy[0].float())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("E,k", [(20, 6), (32, 8), (64, 8), (100, 8), (250, 16), (256, 8)])
+def test_sigmoid_scores_below_the_smallest_normal_number(E, k, normalize, dtype):
+    """Logits from -100 to -84, whose scores pass 2^-126 and are fp32 numbers on the grid of 2^-149: the
+    order of the experts, their weights and gradients are those of the definition.  Such a
+    score is off by its relative error (rel of test_gpu_balanced_routing.py) and, below 2^-126, by
+    3 units of that grid, two of the exponential and one of a product; so are the gradients' terms."""
+    import spark_gpt_b200 as b200
+    from oracle import step_oracle as O
+    from tests.test_gpu_balanced_routing import grad_scale, rel
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.full((9, E), -120.0, device=DEV)
+    for t in range(9):
+        at = torch.randperm(E, device=DEV, generator=g)[:32]
+        x[t, at] = -84.0 - 0.5 * torch.arange(len(at), device=DEV)[torch.randperm(len(at), device=DEV, generator=g)]
+    x = x.to(dtype).requires_grad_(True)
+    w, sel = b200.route_experts(x, k, normalize=normalize)
+    x64 = x.detach().double().requires_grad_(True)
+    ref, ref_sel = O.route(x64, k, None, "sigmoid", 1, 1, "max", normalize, 1.0)
+    assert torch.equal(sel, ref_sel)
+    grid = 3 * 2.0 ** -149 * (1e20 if normalize else 1.0)
+    assert bool(((w.double() - ref).abs() <= rel(E) * ref + grid).all()) and bool((w > 0).all())
+    dw = torch.randn(9, k, device=DEV, generator=g)
+    w.backward(dw)
+    want, = torch.autograd.grad(ref, x64, dw.double())
+    size = grad_scale(O.route_scores(x64.detach(), "sigmoid"), sel, dw, "sigmoid", normalize, 1.0)
+    tol = (2.0 ** -8 if dtype == BF16 else 2.0 ** -23) * want.abs() + rel(E) * size + (
+        grid * (1 + dw.abs().amax()) + (2.0 ** -133 if dtype == BF16 else 2.0 ** -149))
+    assert bool(((x.grad.double() - want).abs() <= tol).all())
