@@ -276,6 +276,23 @@ route_experts_fwd_kernel(const T* __restrict__ logits, long long ld, long long r
             won_s[q] = bias ? sh_s[tok][won_e[q]]
                             : select_value(static_cast<int>(static_cast<unsigned>(mine >> 32) ^ 0x80000000u));
         }
+        if constexpr (L == 16) {
+          // By rank, as the rounds have them: a token's scores are then added in one order, whether
+          // or not the token beside it in the warp took the rounds.
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < SLOTS; ++q)
+            if (won_r[q] < k)
+              sh_list[tok][won_r[q]] = static_cast<unsigned long long>(won_e[q]) << 32 | __float_as_uint(won_s[q]);
+          __syncwarp();
+          const unsigned long long mine = sub < k ? sh_list[tok][sub] : 0ull;
+#pragma unroll
+          for (int q = 0; q < SLOTS; ++q) {
+            won_r[q] = q * L + sub;
+            won_e[q] = q ? 0 : static_cast<int>(mine >> 32);
+            won_s[q] = q ? 0.f : __uint_as_float(static_cast<unsigned>(mine));
+          }
+        }
       }
     }
     if (!ranked) {
