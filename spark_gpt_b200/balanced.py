@@ -57,6 +57,10 @@ def route_experts(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | None
     ("top2").  The weights are the selected scores without the bias, divided by their sum
     (+ 1e-20) with `normalize`, times `scale`.  Differentiable in the logits through the
     weights; the bias has no gradient.  E <= 256, k <= 16, at most 32 groups."""
+    if torch.compiler.is_compiling():
+        return _route_outside_graph(logits, top_k, bias=bias, scoring=scoring, num_groups=num_groups,
+                                    kept_groups=kept_groups, group_score=group_score,
+                                    normalize=normalize, scale=scale)
     if scoring not in SCORINGS:
         raise ValueError(f"route_experts: scoring must be one of {SCORINGS}, got {scoring!r}")
     if group_score not in GROUP_SCORES:
@@ -87,12 +91,17 @@ def route_experts(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | None
     return w.view(*lead, top_k), sel.view(*lead, top_k)
 
 
+_route_outside_graph = ops.outside_graph(route_experts)
+
+
 def balance_bias(bias: torch.Tensor, selected: torch.Tensor, rate: float,
                  group=None) -> torch.Tensor:
     """The next selection bias: bias + rate * sign(mean load - load), a new (E,) fp32 tensor.
 
     A load is the number of times an expert occurs in `selected` (any shape, int64; ids
     outside [0, E) are not counted), summed over the ranks of `group` if one is given."""
+    if torch.compiler.is_compiling():
+        return _balance_outside_graph(bias, selected, rate, group)
     if selected.device != bias.device:
         raise RuntimeError(f"balance_bias: selected must be on {bias.device}, got "
                            f"{selected.device}")
@@ -102,6 +111,9 @@ def balance_bias(bias: torch.Tensor, selected: torch.Tensor, rate: float,
     counts = ops.expert_counts(selected, bias.shape[0])
     dist.all_reduce(counts, group=group)
     return ops.balance_bias(bias.detach(), counts, float(rate))
+
+
+_balance_outside_graph = ops.outside_graph(balance_bias)
 
 
 class _RouterLogitsFn(torch.autograd.Function):
@@ -137,6 +149,11 @@ class _RouterLogitsFn(torch.autograd.Function):
         return dx, dw
 
 
+@ops.outside_graph
+def _module_outside_graph(module, hidden_states):
+    return module.forward(hidden_states)
+
+
 class BalancedRouter(nn.Module):
     """TopKRouter with ``route_experts``'s selection.
 
@@ -166,6 +183,8 @@ class BalancedRouter(nn.Module):
         return self
 
     def forward(self, hidden_states: torch.Tensor):
+        if torch.compiler.is_compiling():
+            return _module_outside_graph(self, hidden_states)
         shape = hidden_states.shape
         logits = _RouterLogitsFn.apply(hidden_states.reshape(-1, shape[-1]), self.weight)
         w, sel = route_experts(
@@ -194,6 +213,8 @@ class BalancedSparseMoE(nn.Module):
         self.experts = Experts(config)
 
     def forward(self, hidden_states: torch.Tensor):
+        if torch.compiler.is_compiling():
+            return _module_outside_graph(self, hidden_states)
         shape = hidden_states.shape
         x = hidden_states.reshape(-1, shape[-1])
         _require_cuda(x)

@@ -23,6 +23,7 @@ def _inf(norm_type) -> bool:
     return norm_type == math.inf
 
 
+@ops.outside_graph
 @torch.no_grad()
 def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     """sqrt of the sum of squares (or, for norm_type inf, the largest magnitude) of all
@@ -34,6 +35,7 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     return ops.grad_clip(None, inf_norm, ops.grad_partials(grads, inf_norm), 0.0)
 
 
+@ops.outside_graph
 @torch.no_grad()
 def clip_grads(grads, max_norm: float, *, out=None, norm_type: float = 2.0) -> torch.Tensor:
     """Scale the gradients by min(1, max_norm / (norm + 1e-6)), in place or into the tensors
@@ -57,6 +59,7 @@ def clip_grads(grads, max_norm: float, *, out=None, norm_type: float = 2.0) -> t
     return ops.clip_grads(grads, dst, inf_norm, float(max_norm))
 
 
+@ops.outside_graph
 @torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, *, sharded=(),
                     group=None) -> torch.Tensor:

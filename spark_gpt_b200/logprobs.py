@@ -58,6 +58,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     `ignore_index` is left out: logprob and entropy 0, alternatives (0, -1), no gradient.
     Any other token outside [0, V) gives NaN.  A -inf logit has probability 0 and no
     gradient; a row of -inf alone has log probabilities -inf, entropy 0 and no gradient."""
+    if torch.compiler.is_compiling():
+        return _outside_graph(logits, tokens, top=top, temperature=temperature,
+                              ignore_index=ignore_index)
     rows = ops.as_rows(logits, "token_logprobs")
     lead = logits.shape[:-1]
     if tokens.shape != lead:
@@ -78,3 +81,6 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
         if top:
             top_lp, top_ids = top_lp.view(*lead, top), top_ids.view(*lead, top)
     return TokenLogprobs(logprob, entropy, top_lp, top_ids)
+
+
+_outside_graph = ops.outside_graph(token_logprobs)

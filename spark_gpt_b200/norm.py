@@ -65,12 +65,17 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
 
     x: bf16 or fp32 CUDA, any leading dimensions and row stride; weight and bias: of the last
     dimension's size, or None.  The result has x's type and shape."""
+    if torch.compiler.is_compiling():
+        return _outside_graph(x, weight, bias, eps)
     if ops.records(x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, eps)
     rows = ops.aligned_rows(ops.as_rows(x, "layer_norm"))
     y, _ = ops.layer_norm_fwd(rows, _param(weight, rows, "weight"), _param(bias, rows, "bias"), eps,
                               False, x)
     return y
+
+
+_outside_graph = ops.outside_graph(layer_norm)
 
 
 class LayerNorm(nn.Module):

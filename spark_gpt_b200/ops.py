@@ -836,6 +836,10 @@ def aligned_rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+# In a traced model the training-step operators run between its graphs: their calls take pointers
+# and streams, which a trace cannot hold.
+outside_graph = torch.compiler.disable
+
 _ENTRIES: dict = {}
 
 

@@ -116,3 +116,63 @@ def test_two_threads_at_once():
     for t in threads:
         t.join()
     assert not wrong
+
+
+class Block(torch.nn.Module):
+    def __init__(self, H=256, E=60, V=259):
+        import spark_gpt_b200 as b200
+        from tests.test_gpu_step_edges import moe
+        super().__init__()
+        self.norm = b200.LayerNorm(H).to(DEV)
+        self.moe = moe(H, E, 4, 128)
+
+    def forward(self, x, tokens):
+        import spark_gpt_b200 as b200
+        out, logits, sel = self.moe(self.norm(x))
+        r = b200.token_logprobs(out, tokens, top=3)
+        w, s = b200.route_experts(out[:, :40], 4, num_groups=4, kept_groups=2)
+        return out, logits, sel, r.logprob, r.entropy, r.top_ids, w, s
+
+
+def test_compiled_model_gives_the_same_bits():
+    """The operators run outside the graphs of a compiled model (a break before and behind each), with
+    their gradients."""
+    torch._dynamo.reset()
+    m = Block()
+    x = torch.randn(70, 256, device=DEV).to(BF16)
+    tokens = torch.randint(256, (70,), device=DEV)
+
+    def run(f, grad):
+        m.zero_grad()
+        with torch.set_grad_enabled(grad):
+            xl = x.clone().requires_grad_(grad)
+            out = f(xl, tokens)
+        if not grad:
+            return list(out)
+        torch.autograd.backward([out[0].sum(), out[3].sum(), out[4].sum(), (out[6] * out[7]).sum()])
+        return [*out, xl.grad, *(p.grad.clone() for p in m.parameters())]
+
+    compiled = torch.compile(m, dynamic=False)
+    for grad in (True, False):
+        for _ in range(2):
+            for a, b in zip(run(m, grad), run(compiled, grad)):
+                assert a.shape == b.shape and torch.equal(a, b)
+
+
+def test_compiled_step_functions():
+    import spark_gpt_b200 as b200
+    torch._dynamo.reset()
+    ps = [torch.nn.Parameter(torch.zeros(n, device=DEV)) for n in (100, 33)]
+    bias = torch.randn(64, device=DEV)
+    sel = torch.randint(64, (100, 4), device=DEV)
+
+    def step(scale):
+        for p in ps:
+            p.grad = torch.full_like(p, 2.0) * scale
+        norm = b200.clip_grad_norm_(ps, 1.0)
+        return norm, b200.grad_norm([p.grad for p in ps]), b200.balance_bias(bias, sel, 0.5) + 0.0
+
+    want = [*step(3.0), *(p.grad for p in ps)]
+    got = [*torch.compile(step)(3.0), *(p.grad for p in ps)]
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
