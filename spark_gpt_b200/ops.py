@@ -1046,18 +1046,21 @@ class GradList:
         devices = set(map(torch.Tensor.get_device, tensors))
         if len(devices) > 1 or -1 in devices:
             raise RuntimeError(f"{name}: the gradients must be CUDA tensors of one device")
-        types = [t.dtype for t in tensors]
-        if not _GRAD_KINDS.keys() >= set(types):
-            raise RuntimeError(f"{name}: expected bf16 or fp32 gradients, got "
-                               f"{(set(types) - _GRAD_KINDS.keys()).pop()}")
+        try:
+            self.kinds = array("i", [_GRAD_KINDS[t.dtype] for t in tensors])
+        except KeyError as e:
+            raise RuntimeError(f"{name}: expected bf16 or fp32 gradients, got {e.args[0]}") from None
         if not all(map(torch.Tensor.is_contiguous, tensors)):
             raise RuntimeError(f"{name}: the gradients must be contiguous")
         if forward_ad._current_level >= 0 and any(
                 forward_ad.unpack_dual(t).tangent is not None for t in tensors):
             raise RuntimeError(f"{name}: it has no forward-mode derivative")
-        self.kinds = array("i", [_GRAD_KINDS[d] for d in types])
         self.ptrs = array("q", list(map(torch.Tensor.data_ptr, tensors)))
         self.sizes = array("q", list(map(torch.Tensor.numel, tensors)))
+
+    def written(self) -> None:
+        """Tell autograd that the tensors were changed in place."""
+        torch.autograd.graph.increment_version(self.tensors)
 
     def args(self):
         return self.ptrs.buffer_info()[0], self.sizes.buffer_info()[0], self.kinds.buffer_info()[0]
@@ -1093,6 +1096,8 @@ def grad_clip(grads: GradList | None, inf_norm: bool, partials, max_norm: float)
         n = len(grads.tensors)
     _call_on(partials, "grad_clip", 1, "b200moe_grad_clip", ptrs, ptrs, sizes, kinds, n, inf_norm,
              partials.data_ptr(), partials.numel(), max_norm, norm.data_ptr())
+    if grads is not None:
+        grads.written()
     return norm
 
 
@@ -1104,4 +1109,5 @@ def clip_grads(grads: GradList, out: GradList, inf_norm: bool, max_norm: float) 
     ptrs, sizes, kinds = grads.args()
     _call_on(first, "clip_grads", 2, "b200moe_clip_grads", ptrs, out.ptrs.buffer_info()[0], sizes,
              kinds, len(grads.tensors), inf_norm, partials.data_ptr(), max_norm, norm.data_ptr())
+    out.written()
     return norm

@@ -232,3 +232,28 @@ def test_statistics_off_their_alignment_are_refused(call):
         call("b200moe_token_logprobs_fwd", 16, 0, 100, 16, 4, 100, 1.0, -100, 0, 16, 16, None, None, 20, None)
     with pytest.raises(RuntimeError, match="stats"):
         call("b200moe_token_logprobs_bwd", 16, 0, 100, 16, 4, 100, 1.0, -100, 20, 16, 16, 16, 16, 100, None)
+
+
+@pytest.mark.parametrize("how", ["clip_grads", "out", "clip_grad_norm_"])
+def test_autograd_sees_that_gradients_were_scaled(monkeypatch, how):
+    """What is scaled in place may be held by a graph (of a penalty on the gradients): its backward is an
+    error then, as after any in-place operation, and is not that of the scaled values."""
+    import spark_gpt_b200 as b200
+    from spark_gpt_b200 import ops
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    monkeypatch.setattr(ops, "_call_on", lambda *args: None)
+    monkeypatch.setattr(ops, "_grad_partials_count", lambda: 592)
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad, other = torch.ones(4), torch.ones(4)
+    penalty = (torch.ones(4, requires_grad=True) * p.grad).sum()
+    result = (torch.ones(4, requires_grad=True) * other).sum()
+    if how == "clip_grads":
+        b200.clip_grads([p.grad], 0.5)
+    elif how == "out":
+        b200.clip_grads([p.grad], 0.5, out=[other])
+    else:
+        b200.clip_grad_norm_([p], 0.5)
+    changed, kept = (result, penalty) if how == "out" else (penalty, result)
+    kept.backward()
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        changed.backward()
