@@ -616,7 +616,8 @@ layer_norm_rows_bwd_kernel(const T* __restrict__ dy, long long ld_dy, const T* _
 }
 
 // ---------------------------------------------------------------------------
-// longer rows: a block goes over its row once for each sum
+// longer rows: a block goes over its row once for each sum, by single elements (2048 x 32768 bf16:
+// 128 us forward, 306 backward; 42 and 62 at the copy bandwidth)
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(kNormThreads)

@@ -12,13 +12,13 @@
 //
 // L lanes take a token (4 to 32), eight consecutive experts a lane, so that a lane's logits are
 // one or two 16-byte loads and 64 experts put four tokens in a warp: what bounds these kernels is
-// instructions (the issue slots are 70-76% busy, DRAM below 15%), and a reduction serves several
-// tokens at once.  Up to 64 experts a lane sorts its keys and k rounds take the largest first
+// instructions (the forward's issue slots are 67-74% busy, the softmax gradient's 64, the sigmoid
+// gradient's 44; DRAM below 15%), and a reduction serves several tokens at once.  Up to 64 experts a lane sorts its keys and k rounds take the largest first
 // key; from 65 on the few keys that reach a bound are listed and ranked (256 experts, top-8:
 // 25 us for 32768 tokens, 34 with the rounds; with 8 lanes a token the bound lets through a third
 // of the keys and the rounds are as fast).  65536 tokens, 64 experts, top-8, softmax, bf16:
-// 21 us forward, 9.6 us backward; 16381 tokens, 256 experts in 8 groups, top-8, sigmoid, fp32: 18 and
-// 7.3 us (25 and 36 MB in all, 3.9 and 5.5 us at the copy bandwidth).
+// 21 us forward, 9.7 us backward; 16381 tokens, 256 experts in 8 groups, top-8, sigmoid, fp32: 19 and
+// 7.4 us (25 and 36 MB in all, 3.9 and 5.5 us at the copy bandwidth).
 #pragma once
 
 #include <climits>

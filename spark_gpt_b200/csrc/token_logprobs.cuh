@@ -27,7 +27,8 @@
 // with twenty alternatives 12 us.
 //
 // Values in masks: a -inf logit has probability 0 and adds nothing to H; a row of -inf alone has
-// log probabilities -inf, H = 0 and no gradient.  A NaN logit makes its row NaN.  A row whose token
+// log probabilities -inf, H = 0 and no gradient; the token's own -inf logit in another row has the
+// gradient g / temperature.  A NaN logit makes its row NaN.  A row whose token
 // is `ignore` is left out: logprob 0, H 0, alternatives (0, -1), gradient 0.  Any other token
 // outside [0, V) gives logprob NaN and a NaN gradient row.  In the pass logits below a floor of
 // about -1e8 / c count as the floor, so that x c - m c, whose product is exact and whose
@@ -487,7 +488,8 @@ __device__ __forceinline__ bool pick_top(const T* __restrict__ row, const Span& 
   return ok;
 }
 
-// The same by one search of the row for each alternative, for any values.
+// The same by one search of the row for each alternative, for any values (4096 x 50257 bf16 with
+// three logits allowed and five alternatives: 850 us, 92 the other way).
 template <int G, typename T>
 __device__ __forceinline__ void pick_top_any(const T* __restrict__ row, int V, int top, int t,
                                              GroupShared<G, true>& sh) {

@@ -56,8 +56,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     Differentiable in the logits through logprob and entropy; the alternatives (the `top` <= 32
     largest logits, equal ones by rising id) are reported only.  A row whose token is
     `ignore_index` is left out: logprob and entropy 0, alternatives (0, -1), no gradient.
-    Any other token outside [0, V) gives NaN.  A -inf logit has probability 0 and no
-    gradient; a row of -inf alone has log probabilities -inf, entropy 0 and no gradient."""
+    Any other token outside [0, V) gives NaN.  A -inf logit has probability 0 and, unless it is the
+    token's, no gradient; a row of -inf alone has log probabilities -inf, entropy 0 and no
+    gradient."""
     if torch.compiler.is_compiling():
         return _outside_graph(logits, tokens, top=top, temperature=temperature,
                               ignore_index=ignore_index)
