@@ -16,6 +16,7 @@ from __future__ import annotations
 import torch
 import torch.distributed as dist
 import torch.nn as nn
+from torch.compiler import is_dynamo_compiling
 
 from . import faults, ops
 from .moe import Experts, _as_bf16, _extra_logit_grad, _require_cuda
@@ -57,7 +58,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | None
     ("top2").  The weights are the selected scores without the bias, divided by their sum
     (+ 1e-20) with `normalize`, times `scale`.  Differentiable in the logits through the
     weights; the bias has no gradient.  E <= 256, k <= 16, at most 32 groups."""
-    if torch.compiler.is_compiling():
+    if is_dynamo_compiling():
         return _route_outside_graph(logits, top_k, bias=bias, scoring=scoring, num_groups=num_groups,
                                     kept_groups=kept_groups, group_score=group_score,
                                     normalize=normalize, scale=scale)
@@ -100,7 +101,7 @@ def balance_bias(bias: torch.Tensor, selected: torch.Tensor, rate: float,
 
     A load is the number of times an expert occurs in `selected` (any shape, int64; ids
     outside [0, E) are not counted), summed over the ranks of `group` if one is given."""
-    if torch.compiler.is_compiling():
+    if is_dynamo_compiling():
         return _balance_outside_graph(bias, selected, rate, group)
     if selected.device != bias.device:
         raise RuntimeError(f"balance_bias: selected must be on {bias.device}, got "
@@ -183,7 +184,7 @@ class BalancedRouter(nn.Module):
         return self
 
     def forward(self, hidden_states: torch.Tensor):
-        if torch.compiler.is_compiling():
+        if is_dynamo_compiling():
             return _module_outside_graph(self, hidden_states)
         shape = hidden_states.shape
         logits = _RouterLogitsFn.apply(hidden_states.reshape(-1, shape[-1]), self.weight)
@@ -213,7 +214,7 @@ class BalancedSparseMoE(nn.Module):
         self.experts = Experts(config)
 
     def forward(self, hidden_states: torch.Tensor):
-        if torch.compiler.is_compiling():
+        if is_dynamo_compiling():
             return _module_outside_graph(self, hidden_states)
         shape = hidden_states.shape
         x = hidden_states.reshape(-1, shape[-1])

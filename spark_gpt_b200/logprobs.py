@@ -14,6 +14,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.compiler import is_dynamo_compiling
 
 from . import ops
 
@@ -59,7 +60,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     Any other token outside [0, V) gives NaN.  A -inf logit has probability 0 and, unless it is the
     token's, no gradient; a row of -inf alone has log probabilities -inf, entropy 0 and no
     gradient."""
-    if torch.compiler.is_compiling():
+    if is_dynamo_compiling():
         return _outside_graph(logits, tokens, top=top, temperature=temperature,
                               ignore_index=ignore_index)
     rows = ops.as_rows(logits, "token_logprobs")

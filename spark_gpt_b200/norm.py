@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.compiler import is_dynamo_compiling
 
 from . import ops
 
@@ -65,7 +66,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
 
     x: bf16 or fp32 CUDA, any leading dimensions and row stride; weight and bias: of the last
     dimension's size, or None.  The result has x's type and shape."""
-    if torch.compiler.is_compiling():
+    if is_dynamo_compiling():
         return _outside_graph(x, weight, bias, eps)
     if ops.records(x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, eps)
